@@ -16,7 +16,6 @@ attends the prefix and itself.  Three operators:
 true, the framework's calls; ``exact`` restates the definitions in 64 bits.
 """
 
-import functools
 import math
 import os
 import random
@@ -36,9 +35,7 @@ _HEADS = [(12, 2, 128), (14, 2, 64), (16, 2, 128), (32, 8, 128), (8, 8, 64)]
 _SECTIONS = {128: "16,24,24", 64: "8,12,12"}
 
 
-@functools.lru_cache(maxsize=None)
 def _engine():
-    """The framework's package, looked up once, as a program that imports it at its top has it."""
     pkg = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "speculative-decoding-lab_b200")
     if pkg not in sys.path:
         sys.path.insert(0, pkg)
@@ -259,7 +256,6 @@ def prepare(case, seed):
             live = torch.tensor([b * new + j for b in range(seqs) for j in range(counts[b])], device=dev)
             grid[live] = flat
             s["slots"] = grid
-            s["pools"] = tuple(x[0].view(-1, hkv, d) for x in (kv._k, kv._v))  # the state that the calls update
         else:
             slots = [tables[b][(starts[b] + j) // _BS] * _BS + (starts[b] + j) % _BS if j < counts[b] else -1
                      for b in range(seqs) for j in range(new)]
@@ -330,7 +326,7 @@ def run(s):
         if s["op"] == "append_rotary":
             kv = s["kv"]
             q = kv.append_rotary(0, s["slots"], s["k"], s["v"], s["table"], s["positions"], s["sections"], query=s["q"])
-            return (q,) + s["pools"]
+            return q, kv._k[0].view(-1, kv.num_kv_heads, kv.head_dim), kv._v[0].view(-1, kv.num_kv_heads, kv.head_dim)
         return engine.paged_attention_shared_prefix(s["q"], s["kv"], 0, s["batch"])
     if s["op"] == "shared_prefix":
         return _attend(s)
