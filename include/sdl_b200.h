@@ -344,8 +344,8 @@ int sdl_prefill_chunk(const sdl_attn_args* args, void* stream);
  * block-table row `prefix_row` and own positions [0, starts[b] + j]; starts
  * may be negative (a row without own keys), and a row with no key at all
  * comes out zero.  Rows j >= valid_rows[b] are not written.  `max_limit`
- * bounds starts[b] + chunk; pages past it are not attended and reported
- * (SDL_DEVERR_BAD_INDEX).  k_new / rope_cos / dense K/V are refused, and the
+ * bounds starts[b] + chunk: a row attends own positions below it only, and a
+ * written row that it cuts off is reported (SDL_DEVERR_BAD_INDEX).  k_new / rope_cos / dense K/V are refused, and the
  * plan fields of `attn` (pages_per_split .. mma_layout, overlap_layers) are
  * not read, except key_count: 0, or the host's sum of starts[b] + chunk.
  * Pool rows that a query row does not attend may hold any value, NaN

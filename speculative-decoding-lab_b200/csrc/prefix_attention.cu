@@ -42,6 +42,7 @@ struct PfxParams {
     const int32_t* starts;
     const int32_t* valid_rows;
     int prefix_row, prefix_len;
+    int max_limit;    // own keys at and past it are not attended
     int B, chunk, Hq, Hkv, ratio, hd;
     int F;            // flat rows of one kv head: B * chunk * ratio
     int row_tile;     // flat rows of one own item
@@ -51,7 +52,7 @@ struct PfxParams {
     int mtiles;       // row tiles of one sequence
     int nsm, mpk;     // own splits (grid bound) and keys of each
     int nslot;        // partial slots of one row: nsp + nsm
-    int own_direct;   // > 0: the merge attends the own keys itself, at most so many
+    int own_direct;   // > 0: the merge attends the own keys itself, at most a page of them
     int p_split;      // 16-bit weights as a hi + lo pair (fp32 output)
     int out_vec;      // out rows take 4-element stores
     float scale_log2;
@@ -62,6 +63,14 @@ struct PfxParams {
 
 SDL_DEV int pfx_nvalid(const PfxParams& p, int b) {
     return p.valid_rows ? max(0, min(p.valid_rows[b], p.chunk)) : p.chunk;
+}
+
+// Own keys that row j of sequence b attends: starts[b] + j + 1, within [0,
+// max_limit].  `over` where the bound cuts some off (the merge reports it).
+SDL_DEV int pfx_limit(const PfxParams& p, int b, int j, bool& over) {
+    const int64_t n = (int64_t)p.starts[b] + j + 1;
+    over = n > p.max_limit;
+    return (int)max((int64_t)0, min(n, (int64_t)p.max_limit));
 }
 
 // One item: flat rows [f0, f1) of kv head g against keys [k0, k1) of the
@@ -97,9 +106,8 @@ SDL_DEV bool pfx_item(const PfxParams& p, int64_t i, Item& it) {
     const int nvalid = pfx_nvalid(p, b);
     const int r0 = t * p.row_tile, r1 = min(R, min(r0 + p.row_tile, nvalid * p.ratio));
     if (r0 >= r1) return false;
-    const int lmax = p.starts[b] + (r1 - 1) / p.ratio + 1;  // keys the tile's last row attends
-    // a length past the grid (max_limit below starts[b] + chunk) is reported
-    if (s == 0 && lmax > p.nsm * p.mpk && threadIdx.x == 0) sdl_raise(p.err, SDL_DEVERR_BAD_INDEX);
+    bool over;
+    const int lmax = pfx_limit(p, b, (r1 - 1) / p.ratio, over);  // keys the tile's last row attends
     it.k0 = s * p.mpk;
     it.k1 = min(lmax, it.k0 + p.mpk);
     it.f0 = b * R + r0;
@@ -124,7 +132,7 @@ SDL_DEV int64_t pfx_page_row(const PfxParams& p, int seq, int pg) {
 // The row of flat index f: its sequence, chunk row, q head and own key limit.
 struct FlatRow {
     int b, j, h, limit;
-    bool valid;
+    bool valid, over;
 };
 
 SDL_DEV FlatRow pfx_prefix_row(const PfxParams& p, int f, int g) {  // limit not set
@@ -134,13 +142,14 @@ SDL_DEV FlatRow pfx_prefix_row(const PfxParams& p, int f, int g) {  // limit not
     r.b = bj / p.chunk;
     r.j = bj - r.b * p.chunk;
     r.limit = 0;
+    r.over = false;
     r.valid = r.j < pfx_nvalid(p, r.b);
     return r;
 }
 
 SDL_DEV FlatRow pfx_row(const PfxParams& p, int f, int g) {
     FlatRow r = pfx_prefix_row(p, f, g);
-    r.limit = max(0, p.starts[r.b] + r.j + 1);
+    r.limit = pfx_limit(p, r.b, r.j, r.over);
     return r;
 }
 
@@ -1516,9 +1525,7 @@ template <int LANES>
 SDL_DEV void merge_own(const PfxParams& p, const FlatRow& r, int g, int d0, int first, int step, MergeState& s) {
     constexpr int U = 4;
     const uint32_t group = LANES == 32 ? 0xffffffffu : 0xffffu << (threadIdx.x & 16);  // the row's lanes
-    const int n = min(r.limit, p.own_direct);
-    // a length past max_limit is reported
-    if (r.limit > p.own_direct && d0 == 0) sdl_raise(p.err, SDL_DEVERR_BAD_INDEX);
+    const int n = r.limit;
     if (first >= n) return;
     const int64_t at = (pfx_page_row(p, p.rows[r.b], 0) * p.Hkv + g) * p.hd + d0;
     const uint16_t* k = reinterpret_cast<const uint16_t*>(p.k_pool) + at;
@@ -1626,6 +1633,7 @@ __global__ void __launch_bounds__(kMergeWarps * 32) prefix_merge_kernel(const __
     // complete before they ran; the partials only now
     pdl_wait();
     pdl_launch_dependents();
+    if (in && r.valid && r.over && lane % LANES == 0) sdl_raise(p.err, SDL_DEVERR_BAD_INDEX);
     if (WARPS == 1 && !(in && r.valid)) return;
     const int d0 = (lane % LANES) * 4;
     const float* op = p.o_part + w * p.nslot * HD + d0;
@@ -1687,6 +1695,7 @@ __global__ void __launch_bounds__(kMergeWarps * 32) prefix_merge_any_kernel(cons
     const int g = (int)(w / p.F), f = (int)(w - (int64_t)g * p.F);
     const FlatRow r = pfx_row(p, f, g);
     if (!r.valid) return;
+    if (r.over && lane == 0) sdl_raise(p.err, SDL_DEVERR_BAD_INDEX);
     const int ns = p.nsp + min(p.nsm, (r.limit + p.mpk - 1) / p.mpk);
     const int64_t idx0 = w * p.nslot;
     float M = -INFINITY;
@@ -1843,6 +1852,7 @@ int make_plan(const sdl_prefix_args* x, Plan& pl) {
     p.block_size = a->block_size; p.table_rows = x->table_rows;
     p.rows = a->rows; p.starts = a->starts; p.valid_rows = a->valid_rows;
     p.prefix_row = x->prefix_row; p.prefix_len = x->prefix_len;
+    p.max_limit = std::max(0, a->max_limit);
     p.B = a->B; p.chunk = a->chunk; p.Hq = a->Hq; p.Hkv = a->Hkv; p.ratio = a->Hq / a->Hkv; p.hd = a->head_dim;
     p.scale_log2 = a->scale * kLog2e;
     p.err = a->err;
@@ -1871,7 +1881,7 @@ int make_plan(const sdl_prefix_args* x, Plan& pl) {
     p.mtiles = cdiv(a->chunk * p.ratio, p.row_tile);
     const int64_t ptiles = (int64_t)p.ptiles * p.Hkv;
     const int64_t mtiles = (int64_t)p.mtiles * p.Hkv * std::max(1, a->B);
-    const int span = std::max(0, a->max_limit);
+    const int span = p.max_limit;
     // mean own keys of a sequence (the bound where the host gives no count)
     const int64_t mean = a->key_count > 0 && a->B > 0 ? std::min<int64_t>(span, a->key_count / a->B + 1) : span;
     const int page = pl.kernel == 1 ? 1 : kPage;

@@ -448,7 +448,9 @@ class SharedPrefixBatch(AttnBatch):
     The prefix is sequence ``prefix_id`` of the cache (its own pages, any
     length); ``rows`` / ``starts`` / ``max_limit`` describe the members' OWN
     pages and positions, which begin at 0 behind the prefix.  ``starts[b]``
-    may be negative down to ``-chunk``: rows without own keys.
+    may be negative down to ``-chunk``: rows without own keys.  Rows attend
+    own positions below ``max_limit`` only; one that it cuts off is reported
+    by the cache's ``check_errors``.
     """
 
     __slots__ = ("prefix_id", "prefix_len", "_plans")

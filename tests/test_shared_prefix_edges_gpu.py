@@ -1,0 +1,82 @@
+"""Edges of the attention over a shared prefix: bounds below a sequence's
+length, masked values at the type's ends, outputs that overlap, plans of very
+many rows.  Definition and tolerances as in ``test_shared_prefix_gpu``.
+"""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from engine.attention import SharedPrefixBatch, paged_attention_shared_prefix
+from test_shared_prefix_gpu import BF, DEV, F32, HF, _build, _check, _exact, _query
+
+pytestmark = pytest.mark.gpu
+
+
+def _i32(*values):
+    return torch.tensor(values, dtype=torch.int32, device=DEV)
+
+
+def _exact_bounded(q, kv, P, starts, bound):
+    """``_exact`` where row j attends min(starts[b] + j + 1, bound) own keys."""
+    rows = [_exact(q[:, j:j + 1], kv, 0, P, [max(-1, min(s + j, bound - 1)) for s in starts])
+            for j in range(q.shape[1])]
+    return tuple(torch.cat(x, 1) for x in zip(*rows))
+
+
+# (kernel, chunk, d, page size, type): CUDA cores narrow and wide and of another
+# head_dim (a lane per dim in the merge), mma.sync, tcgen05 with own items of
+# both kinds, the plan's own choice
+FORMS = [(1, 4, 64, 4, F32), (1, 30, 64, 16, F32), (1, 4, 20, 16, HF), (2, 4, 128, 16, BF), (2, 9, 64, 16, HF),
+         (3, 4, 128, 16, BF), (3, 33, 128, 16, HF), (0, 4, 128, 16, BF), (0, 40, 64, 16, BF)]
+
+
+@pytest.mark.parametrize("form", FORMS, ids=str)
+@pytest.mark.parametrize("split", [0, 16, 1000])
+def test_a_bound_below_a_length_cuts_the_keys_and_is_reported(form, split):
+    kernel, chunk, d, bs, dtype = form
+    P, owns = 64, [130, 80]
+    kv, g = _build(P, owns, 2, d, bs, dtype, 3)
+    q = _query(g, 2, chunk, 8, d, dtype)
+    starts = [n - chunk for n in owns]
+    w = dtype if dtype != F32 else None
+
+    def call(starts, bound, valid=None):
+        return paged_attention_shared_prefix(q, kv, 0, SharedPrefixBatch(0, P, _i32(1, 2), _i32(*starts), bound, valid),
+                                             kernel=kernel, own_split=split)
+
+    for use, bound in ((starts, 111), (starts, 129), (starts, 1), (starts, 0), ([2 ** 31 - 1, starts[1]], 130),
+                       ([2 ** 31 - 3, -chunk], 100)):
+        got = call(use, bound)
+        _check(got, _exact_bounded(q, kv, P, use, bound), w)
+        with pytest.raises(RuntimeError, match="0x4"):
+            kv.check_errors()
+    for use, bound in ((starts, 130), (starts, 200), ([-2 ** 31, starts[1]], 80), ([-chunk, -chunk], 0)):
+        _check(call(use, bound), _exact_bounded(q, kv, P, use, bound), w)
+        kv.check_errors()
+    # rows past valid_rows are not written and not reported
+    got = call(starts, starts[0] + 2, _i32(2, chunk))
+    exact = _exact_bounded(q, kv, P, starts, starts[0] + 2)
+    _check(got[0, :2], tuple(x[0, :2] for x in exact), w)
+    _check(got[1], tuple(x[1] for x in exact), w)
+    kv.check_errors()
+
+
+@pytest.mark.parametrize("d,hq", [(128, 12), (64, 6)])
+def test_a_bound_below_a_length_where_the_merge_attends(d, hq):
+    """Sequences with at most a page of own keys, many of them."""
+    B, chunk = 170, 2
+    kv, g = _build(50, [8] * B, 2, d, 16, BF, 2)
+    q = _query(g, B, chunk, hq, d, BF)
+    rows = torch.arange(1, B + 1, dtype=torch.int32, device=DEV)
+    for P in (50, 0):
+        for starts, bound, bad in (([6] * B, 5, True), ([6] * B, 8, False), ([2 ** 31 - 1] + [6] * (B - 1), 8, True),
+                                   ([6] * B, 0, True)):
+            batch = SharedPrefixBatch(0, P, rows, _i32(*starts), bound)
+            _check(paged_attention_shared_prefix(q, kv, 0, batch), _exact_bounded(q, kv, P, starts, bound), BF)
+            if bad:
+                with pytest.raises(RuntimeError, match="0x4"):
+                    kv.check_errors()
+            else:
+                kv.check_errors()
