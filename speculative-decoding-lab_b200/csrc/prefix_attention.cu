@@ -1083,15 +1083,17 @@ SDL_DEV float max3_nan(float a, float b, float c) {
 }
 
 // 2^x of a pair on the FMA pipe, for 16-bit weights: x = n + f with n the
-// nearest integer (adding 1.5 * 2^23 leaves it in the low mantissa bits) and
-// |f| <= 1/2, 2^f by the degree-4 minimax polynomial of that interval (relative
-// error 2^-18.4 in fp32, fitted with the Remez exchange), n added to the
-// exponent.  x is clamped at -126: smaller weights come out as 2^-126,
-// as does a NaN's (the caller's running maximum carries those).
+// nearest integer (adding 1.5 * 2^23 + 127 leaves n + 127 in the low mantissa
+// bits) and |f| <= 1/2, 2^f by the degree-4 minimax polynomial of that interval
+// (relative error 2^-18.4 in fp32, fitted with the Remez exchange), times 2^n,
+// whose exponent field is n + 127.  x is clamped at -127, where that field, and
+// the weight, is zero: a masked key weighs nothing, whatever its value is.  So
+// does a NaN (the caller's running maximum carries those).
 SDL_DEV void ex2_poly2(float& a, float& b) {
-    const uint64_t magic = pack_f32x2(12582912.f, 12582912.f), minus = pack_f32x2(-12582912.f, -12582912.f);
+    constexpr float kMagic = 12582912.f + 127.f;
+    const uint64_t magic = pack_f32x2(kMagic, kMagic), minus = pack_f32x2(-kMagic, -kMagic);
     const uint64_t neg = pack_f32x2(-1.f, -1.f);
-    const uint64_t x = pack_f32x2(fmaxf(a, -126.f), fmaxf(b, -126.f));
+    const uint64_t x = pack_f32x2(fmaxf(a, -127.f), fmaxf(b, -127.f));
     const uint64_t t = add_f32x2(x, magic);
     const uint64_t f = fma_f32x2(add_f32x2(t, minus), neg, x);
     uint64_t r = pack_f32x2(0.009570102f, 0.009570102f);
@@ -1099,11 +1101,10 @@ SDL_DEV void ex2_poly2(float& a, float& b) {
     r = fma_f32x2(r, f, pack_f32x2(0.24024744f, 0.24024744f));
     r = fma_f32x2(r, f, pack_f32x2(0.6931218f, 0.6931218f));
     r = fma_f32x2(r, f, pack_f32x2(0.9999993f, 0.9999993f));
-    float r0, r1, t0, t1;
-    unpack_f32x2(r, r0, r1);
+    float t0, t1;
     unpack_f32x2(t, t0, t1);
-    a = __int_as_float(__float_as_int(r0) + (__float_as_int(t0) << 23));
-    b = __int_as_float(__float_as_int(r1) + (__float_as_int(t1) << 23));
+    r = fma_f32x2(r, pack_f32x2(__int_as_float(__float_as_int(t0) << 23), __int_as_float(__float_as_int(t1) << 23)), 0ull);
+    unpack_f32x2(r, a, b);
 }
 
 template <int HD, typename T, int TILES, bool kOwn>
@@ -1554,11 +1555,10 @@ SDL_DEV void merge_own(const PfxParams& p, const FlatRow& r, int g, int d0, int 
 
 // The slots of row w from `first`, `per` side by side, every `step`, once more,
 // its own ranges key by key.  An item multiplies every V row of its keys by every
-// query row's weights, and the weight 0 (or 2^-126, the least one that ex2_poly2
-// returns) of a key behind a row's limit times an infinity or a NaN is not 0: a
-// row whose values came out so while its sum did not is joined again without the
-// keys that it does not attend.  `lanes` lanes hold the row, dims d0 + i * dstep
-// each.
+// query row's weights, and the weight 0 of a key behind a row's limit times an
+// infinity or a NaN is not 0: a row whose values came out so while its sum did
+// not is joined again without the keys that it does not attend.  `lanes` lanes
+// hold the row, dims d0 + i * dstep each.
 template <int ND>
 SDL_DEV void merge_again(const PfxParams& p, const FlatRow& r, int g, int64_t w, int ns, int first, int per, int step,
                          int d0, int dstep, int lanes, uint32_t group, float& m, float& l, float (&o)[ND]) {

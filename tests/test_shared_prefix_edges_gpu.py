@@ -9,7 +9,7 @@ import pytest
 import torch
 
 from engine.attention import SharedPrefixBatch, paged_attention_shared_prefix
-from test_shared_prefix_gpu import BF, DEV, F32, HF, _build, _check, _exact, _query
+from test_shared_prefix_gpu import BF, DEV, F32, HF, PLANTS, _build, _check, _exact, _planted, _query
 
 pytestmark = pytest.mark.gpu
 
@@ -80,3 +80,49 @@ def test_a_bound_below_a_length_where_the_merge_attends(d, hq):
                     kv.check_errors()
             else:
                 kv.check_errors()
+
+
+def _large(dtype):
+    """A value of which 2^-126 would still move a row."""
+    return 60000.0 if dtype == HF else 2.0 ** 126
+
+
+@pytest.mark.parametrize("case", PLANTS, ids=str)
+def test_a_large_value_behind_a_row_weighs_nothing(case):
+    """The largest values of a chunk's later rows do not reach the earlier
+    ones, in any column of a tile."""
+    kernel, P, before, chunk, d, bs, dtype = case
+    kv, batch, q, exact, places = _planted(case, False)
+    w = dtype if dtype != F32 else None
+    for pos, page, at in places:
+        kept = kv._v[0, page, at, 1].clone()
+        kv._v[0, page, at, 1] = _large(dtype)
+        got = paged_attention_shared_prefix(q, kv, 0, batch, kernel=kernel)
+        kv._v[0, page, at, 1] = kept
+        first = pos - before
+        _check(got[0, :first], tuple(x[0, :first] for x in exact), w) if first else None
+        _check(got[0, :, :4], tuple(x[0, :, :4] for x in exact), w)
+        _check(got[1], tuple(x[1] for x in exact), w)
+    kv.check_errors()
+
+
+@pytest.mark.parametrize("case", PLANTS, ids=str)
+@pytest.mark.parametrize("prefix", [True, False])
+@pytest.mark.parametrize("score", [-16.0, float("-inf")])
+def test_a_large_value_of_a_key_far_below_weighs_nothing(case, prefix, score):
+    """A key whose weight lies below fp32's range, or whose score is -inf."""
+    kernel, P, before, chunk, d, bs, dtype = case
+    kv, batch, q, exact, places = _planted(case, prefix)
+    w = dtype if dtype != F32 else None
+    q[..., 4:, :] = q[..., 4:, :].abs() + 0.5  # of kv head 1: scores of -16 sum q / sqrt(d) < -100
+    for pos, page, at in places:
+        kept = kv._k[0, page, at, 1].clone(), kv._v[0, page, at, 1].clone()
+        kv._k[0, page, at, 1] = score
+        kv._v[0, page, at, 1] = _large(dtype)
+        got = paged_attention_shared_prefix(q, kv, 0, batch, kernel=kernel)
+        kv._v[0, page, at, 1] = 0.0
+        kv._k[0, page, at, 1] = -16.0  # the scores' rounding bound needs a finite one
+        want = _exact(q, kv, 0, P, [before, before])
+        kv._k[0, page, at, 1], kv._v[0, page, at, 1] = kept
+        _check(got, want, w)
+    kv.check_errors()
