@@ -62,15 +62,19 @@ SDL_DEV int axis_of_pair(const RopeParams& p, int pair) {
 }
 
 // cos / sin of `n` consecutive pairs from `pair`; false when a position lies
-// outside the table (the angles are then NaN).
+// outside the table (the angles of its pairs are then NaN).
 template <int n>
 SDL_DEV bool load_angles(const RopeParams& p, int t, int pair, float (&c)[n], float (&s)[n]) {
     const int a0 = axis_of_pair(p, pair);
+    const float nan = __int_as_float(0x7fc00000);
     bool ok = true;
     if (a0 == axis_of_pair(p, pair + n - 1)) {
         const int64_t pos = rope_position(p, a0, t);
         ok = pos >= 0 && pos < p.table_rows;
-        if (ok) {
+        if (!ok) {
+#pragma unroll
+            for (int e = 0; e < n; ++e) c[e] = s[e] = nan;
+        } else {
             const float* row = p.table + pos * 2 * p.R + pair;
 #pragma unroll
             for (int e = 0; e < n; e += 4) {
@@ -86,13 +90,9 @@ SDL_DEV bool load_angles(const RopeParams& p, int t, int pair, float (&c)[n], fl
             const int64_t pos = rope_position(p, axis_of_pair(p, pair + e), t);
             const bool in = pos >= 0 && pos < p.table_rows;
             ok = ok && in;
-            c[e] = in ? __ldg(p.table + pos * 2 * p.R + pair + e) : 0.f;
-            s[e] = in ? __ldg(p.table + (pos * 2 + 1) * p.R + pair + e) : 0.f;
+            c[e] = in ? __ldg(p.table + pos * 2 * p.R + pair + e) : nan;
+            s[e] = in ? __ldg(p.table + (pos * 2 + 1) * p.R + pair + e) : nan;
         }
-    }
-    if (!ok) {
-#pragma unroll
-        for (int e = 0; e < n; ++e) c[e] = s[e] = __int_as_float(0x7fc00000);
     }
     return ok;
 }

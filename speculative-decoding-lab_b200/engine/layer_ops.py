@@ -219,8 +219,8 @@ def rope_axes(q: torch.Tensor, k: Optional[torch.Tensor], table: torch.Tensor, p
     each axis turns, in order: pair ``i`` (dims ``i`` and ``i + R/2``) of row
     ``t`` turns by ``table[positions[axis of i, t], :, i]``.  The arithmetic
     is fp32, rounded once (``rope_`` keeps the framework chain's roundings
-    instead).  A pair whose position lies outside the table comes out NaN (a
-    16-byte piece of pairs at a time).
+    instead).  A pair whose position lies outside the table comes out NaN, the
+    row's other pairs as usual.
 
     ``out = (q_out, k_out)`` receives the result (rows of back-to-back heads;
     they may be ``q`` and ``k`` themselves).
