@@ -538,7 +538,8 @@ int sdl_swiglu(const void* x, int64_t x_row_stride, void* out, int64_t out_row_s
  * rows: engine/model.py:50-56).  Pair i of a row (dims i and i + rotary/2)
  * turns by table[positions[axis of i][t]][0/1][i]; the axes' sections hold
  * consecutive pairs.  fp32 arithmetic, rounded once; dims past `rotary` are
- * copied.  A pair whose position lies outside the table comes out NaN.
+ * copied.  A pair whose position lies outside the table comes out NaN and is
+ * reported in `err`, where given (SDL_DEVERR_BAD_INDEX).
  * ------------------------------------------------------------------- */
 typedef struct sdl_rope_args {
     const void* q; int64_t q_row_stride;         /* [T][Hq][d]; NULL with Hq 0 */

@@ -206,7 +206,7 @@ __global__ void __launch_bounds__(256, 3) rope_vec_kernel(const RopeParams p) {
                 const int64_t pos = rope_position(p, ax, t);
                 ok = ok && pos >= 0 && pos < p.table_rows;
             }
-        if (!ok && first) sdl_raise(p.err, SDL_DEVERR_BAD_INDEX);
+        if (!ok && threadIdx.y == 0) sdl_raise(p.err, SDL_DEVERR_BAD_INDEX);
     }
 #pragma unroll
     for (int u = 0; u < kHeadsPerThread; ++u) {
@@ -256,6 +256,7 @@ __global__ void __launch_bounds__(256) rope_scalar_kernel(const RopeParams p) {
         } else if (e < half && head_turns(p, h)) {
             const int64_t pos = rope_position(p, axis_of_pair(p, e), t);
             const bool in = pos >= 0 && pos < p.table_rows;
+            if (!in && h == 0) sdl_raise(p.err, SDL_DEVERR_BAD_INDEX);
             const float c = in ? __ldg(p.table + pos * 2 * p.R + e) : __int_as_float(0x7fc00000);
             const float s = in ? __ldg(p.table + (pos * 2 + 1) * p.R + e) : __int_as_float(0x7fc00000);
             const float2 r = turn(to_f32<T>(src[e]), to_f32<T>(src[e + half]), c, s);

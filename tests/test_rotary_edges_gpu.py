@@ -48,3 +48,38 @@ def test_a_bad_position_spoils_its_own_pairs_alone(dtype, d, rotary, sections):
     assert torch.equal(turned.nan_to_num(9.0), got[0].nan_to_num(9.0))
     rows = kv._k[0].view(-1, 2, d)[slots.long()]
     assert (rows[:-1] == 0).all() and torch.equal(rows[-1], want[1][-1])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("d,rotary,sections", SPLITS)
+@pytest.mark.parametrize("heads", [(3, 2), (0, 2)])
+def test_the_c_entry_reports_a_bad_position_of_any_axis(dtype, d, rotary, sections, heads):
+    import ctypes
+
+    from engine import _lib
+
+    axes = len(sections)
+    q, k, _, table, pos = _inputs(3, 3, 2, d, dtype, axes, 50, d, rotary)
+    q, k, pos = q.contiguous(), k.contiguous(), pos.contiguous()
+    err = torch.zeros(1, dtype=torch.int32, device=DEV)
+    a = _lib.SdlRopeArgs()
+    if heads[0]:
+        a.q = a.q_out = q.data_ptr()
+        a.q_row_stride = a.q_out_row_stride = 3 * d
+    a.k = a.k_out = k.data_ptr()
+    a.k_row_stride = a.k_out_row_stride = 2 * d
+    a.table, a.table_rows, a.positions, a.pos_stride, a.pos64 = table.data_ptr(), 50, pos.data_ptr(), 3, 1
+    a.err, a.axes, a.num_tokens, a.head_dim, a.rotary = err.data_ptr(), axes, 3, d, rotary
+    a.Hq, a.Hkv, a.dtype = heads[0], heads[1], _lib.dtype_code(dtype)
+    for i, n in enumerate(sections):
+        a.sections[i] = n
+    _lib.check(_lib.load().sdl_rope_axes(ctypes.byref(a), _lib.stream_handle(DEV)), "sdl_rope_axes")
+    assert int(err) == 0
+    for axis, n in enumerate(sections):
+        for row, value in ((0, 50), (2, -1)):
+            kept = pos[axis, row].clone()
+            pos[axis, row] = value
+            err.zero_()
+            _lib.check(_lib.load().sdl_rope_axes(ctypes.byref(a), _lib.stream_handle(DEV)), "sdl_rope_axes")
+            assert int(err) == (0x4 if n else 0)  # an axis without pairs turns nothing
+            pos[axis, row] = kept
