@@ -156,8 +156,10 @@ def _check_heads(x: torch.Tensor, name: str, tokens: int, heads: Optional[int], 
 
 
 def _has_head_rows(x: torch.Tensor) -> bool:
-    """Unit-stride, back-to-back heads (rows may be strided)."""
-    return (x.stride(2) == 1 or x.shape[2] == 1) and (x.stride(1) == x.shape[2] or x.shape[1] == 1)
+    """Unit-stride, back-to-back heads (rows may be strided).  A tensor without
+    elements has them whatever its strides, which a copy would keep."""
+    return x.numel() == 0 or (
+        (x.stride(2) == 1 or x.shape[2] == 1) and (x.stride(1) == x.shape[2] or x.shape[1] == 1))
 
 
 def _check_out_rows(x: torch.Tensor, name: str) -> None:

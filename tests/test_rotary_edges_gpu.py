@@ -83,3 +83,26 @@ def test_the_c_entry_reports_a_bad_position_of_any_axis(dtype, d, rotary, sectio
             _lib.check(_lib.load().sdl_rope_axes(ctypes.byref(a), _lib.stream_handle(DEV)), "sdl_rope_axes")
             assert int(err) == (0x4 if n else 0)  # an axis without pairs turns nothing
             pos[axis, row] = kept
+
+
+@pytest.mark.parametrize("heads", [1, 2, 5])
+def test_empty_calls_of_sliced_tensors(heads):
+    """No tokens, with the strides of a slice; no heads."""
+    q, k, v, table, pos = _inputs(4, heads, 2, 64, torch.bfloat16, 1, 50, 1, rotary=32)
+    wide = torch.zeros((4, heads, 128), dtype=q.dtype, device=DEV)[..., :64]
+    pair = torch.zeros((4, 2, 128), dtype=q.dtype, device=DEV)[:, :, ::2]
+    kv = _cache(2, 64, torch.bfloat16, [4])
+    slots = kv.reserve([0], [0], [4])[:0]
+    for a in (wide[:0], q[:0], wide.transpose(0, 1)[:, :0].transpose(0, 1)):
+        for b in (pair[:0], k[:0]):
+            out = layer_ops.rope_axes(a, b, table, pos[:0])
+            assert out[0].shape == (0, heads, 64) and out[1].shape == (0, 2, 64)
+            given = torch.empty_like(q[:0]), torch.empty_like(k[:0])
+            assert layer_ops.rope_axes(a, b, table, pos[:0], out=given)[0] is given[0]
+            assert kv.append_rotary(0, slots, b, b, table, pos[:0], query=a).shape == (0, heads, 64)
+            assert kv.append_rotary(0, slots, b, pair[:0], table, pos[:0]) is None
+    none = wide[:, :0]
+    turned, other = layer_ops.rope_axes(none, k, table, pos)
+    assert turned.shape == (4, 0, 64)
+    _check(other, k, table, pos, None)
+    kv.check_errors()
