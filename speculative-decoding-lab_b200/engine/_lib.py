@@ -288,6 +288,66 @@ def ptr(t: Optional[torch.Tensor]) -> Optional[int]:
     return None if t is None else t.data_ptr()
 
 
+# ------------------------------------------------------------ shared memory
+def _runs(t: torch.Tensor):
+    """``t`` as runs of back-to-back elements: the dims over the runs as
+    (size, stride) pairs, and a run's length in elements."""
+    dims = [(n, st) for n, st in zip(t.shape, t.stride()) if n > 1]
+    run = 1
+    while dims and dims[-1][1] == run:
+        run *= dims.pop()[0]
+    return dims, run
+
+
+def _run_addresses(t: torch.Tensor, dims) -> torch.Tensor:
+    at = torch.tensor([t.data_ptr()], dtype=torch.int64, device="cpu")
+    for n, st in dims:
+        step = torch.arange(n, dtype=torch.int64, device="cpu") * (st * t.element_size())
+        at = (at[:, None] + step).reshape(-1)
+    return at.sort().values
+
+
+def overlaps_itself(t: torch.Tensor) -> bool:
+    """Whether two elements of ``t`` share memory."""
+    if t.numel() == 0:
+        return False
+    dims, run = _runs(t)
+    reach = run  # elements that the dims so far span
+    for n, st in sorted(dims, key=lambda x: x[1]):
+        if st < reach:
+            break
+        reach += (n - 1) * st
+    else:
+        return False
+    at = _run_addresses(t, dims)
+    return bool((at.diff() < run * t.element_size()).any())
+
+
+def share_memory(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether an element of ``a`` and one of ``b`` share memory: by their
+    whole spans where those are apart, else run by run."""
+    if a.numel() == 0 or b.numel() == 0:
+        return False
+    lo_a, lo_b = a.data_ptr(), b.data_ptr()
+    end_a, end_b = (
+        lo + (sum((n - 1) * st for n, st in zip(t.shape, t.stride())) + 1) * t.element_size()
+        for lo, t in ((lo_a, a), (lo_b, b)))
+    if end_a <= lo_b or end_b <= lo_a:
+        return False
+    (dims_a, run_a), (dims_b, run_b) = _runs(a), _runs(b)
+    at_a, at_b = _run_addresses(a, dims_a), _run_addresses(b, dims_b)
+    # the first run of b that ends behind each start in a: does it begin before that run of a ends?
+    i = torch.searchsorted(at_b, at_a - run_b * b.element_size(), right=True)
+    found = i < at_b.numel()
+    return bool((at_b[i[found]] < at_a[found] + run_a * a.element_size()).any())
+
+
+def same_elements(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether ``a`` and ``b``, of one shape, are the same elements in place."""
+    return a.data_ptr() == b.data_ptr() and a.dtype == b.dtype and all(
+        x == y for n, x, y in zip(a.shape, a.stride(), b.stride()) if n > 1)
+
+
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 # the current device's index, for callers that hold a CUDA tensor (so CUDA is initialised)
 current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)

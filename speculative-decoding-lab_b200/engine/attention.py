@@ -497,7 +497,7 @@ class _PrefixPlan:
     flags, thread) combination; later calls update the pointers and the
     layer."""
 
-    __slots__ = ("args", "attn", "ref", "ws_floats", "out_dtype", "zero", "dense", "kv", "table")
+    __slots__ = ("args", "attn", "ref", "ws_floats", "out_dtype", "zero", "dense", "kv", "table", "gap")
 
     def __init__(self, q, kv, batch, out, out_dtype, kernel, prefix_split, own_split) -> None:
         self.kv = weakref.ref(kv)  # the struct points at the cache's tensor maps
@@ -506,6 +506,7 @@ class _PrefixPlan:
         self.dense = q.is_contiguous()
         self.out_dtype = out.dtype if out is not None else out_dtype or q.dtype
         self.ws_floats = 0
+        self.gap = None  # distance of the last checked output from its query
         shaped = out
         if shaped is None:  # the strides and alignment of a new tensor
             shaped = torch.empty(q.shape, dtype=self.out_dtype, device=kv.device)
@@ -539,6 +540,8 @@ def _check_prefix_call(q, kv, batch, out, out_dtype) -> None:
         raise ValueError("out must be {} on {} with unit-stride rows".format(tuple(q.shape), dev))
     if out is not None and any(n > 1 and st == 0 for n, st in zip(out.shape, out.stride())):
         raise ValueError("out must not be a broadcast tensor")
+    if out is not None and _lib.overlaps_itself(out):
+        raise ValueError("out's rows must not overlap")
 
 
 def _prefix_args(q, kv, layer, batch, out, kernel, prefix_split, own_split) -> _lib.SdlPrefixArgs:
@@ -583,7 +586,8 @@ def paged_attention_shared_prefix(
     prefix).  The rows' own K/V must be stored already (``append`` or
     ``append_rotary``, the latter with positions ``prefix_len + own``).  A row
     with no key at all comes out zero; rows past ``valid_rows`` are left as
-    they are in ``out`` (zero in a new one).
+    they are in ``out`` (zero in a new one).  ``out`` may be ``q`` itself; an
+    ``out`` that overlaps it, or itself, otherwise is refused.
 
     Scratch memory comes from torch's allocator on the current stream, so
     calls on several streams and captured graphs do not share any.
@@ -626,6 +630,12 @@ def paged_attention_shared_prefix(
             out = torch.empty_like(q) if plan.dense else torch.empty_like(q, memory_format=torch.contiguous_format)
         else:
             out = torch.empty(q.shape, dtype=plan.out_dtype, device=dev)
+    else:
+        gap = out.data_ptr() - q.data_ptr()
+        if gap != plan.gap:
+            if not _lib.same_elements(out, q) and _lib.share_memory(out, q):
+                raise ValueError("out must be the query itself or not overlap it")
+            plan.gap = gap
     if not plan.ws_floats:
         return out
     ws = torch.empty(plan.ws_floats, dtype=torch.float32, device=dev)

@@ -23,3 +23,52 @@ def test_layouts_that_a_rotation_takes(shape, index, want):
     x = torch.zeros(shape)[index]
     assert layer_ops._has_head_rows(x) is want
     assert layer_ops._has_head_rows(x.contiguous())
+
+
+def _bytes(t):
+    """Addresses of every byte of ``t``, with repetitions."""
+    import itertools
+
+    out = []
+    for at in itertools.product(*(range(n) for n in t.shape)):
+        a = t.data_ptr() + t.element_size() * sum(i * st for i, st in zip(at, t.stride()))
+        out += range(a, a + t.element_size())
+    return out
+
+
+def test_shared_memory_is_found_byte_by_byte():
+    import random
+
+    from engine import _lib
+
+    rng = random.Random(5)
+    buf = torch.zeros(400, dtype=torch.bfloat16)
+    seen = {True: 0, False: 0}
+    alone = {True: 0, False: 0}
+
+    def view():
+        base = buf if rng.random() < 0.7 else buf.view(torch.float32)
+        while True:
+            shape = [rng.randint(0 if rng.random() < 0.1 else 1, 4) for _ in range(rng.randint(1, 4))]
+            stride = [rng.choice([0, 1, 2, 3, 4, 5, 8, 12, 16, 24, 40]) for _ in shape]
+            if rng.random() < 0.7:
+                stride[-1] = 1
+            at = rng.randint(0, 60)
+            if at + sum(max(0, n - 1) * st for n, st in zip(shape, stride)) < base.numel():
+                return base.as_strided(shape, stride, at)
+
+    for _ in range(1500):
+        a, b = view(), view()
+        x, y = _bytes(a), _bytes(b)
+        assert _lib.overlaps_itself(a) is (len(set(x)) < len(x)), (a.shape, a.stride())
+        assert _lib.share_memory(a, b) is bool(set(x) & set(y)), (a.shape, a.stride(), b.shape, b.stride())
+        alone[_lib.overlaps_itself(a)] += 1
+        seen[_lib.share_memory(a, b)] += 1
+    assert min(seen.values()) > 200 and min(alone.values()) > 200
+    # column blocks of one wider tensor interleave and share nothing
+    wide = torch.zeros(50, 24)
+    assert not _lib.share_memory(wide[:, :8], wide[:, 8:16])
+    assert _lib.share_memory(wide[:, :9], wide[:, 8:16])
+    q = wide[:, :8]
+    assert _lib.same_elements(q, q.view(50, 8)) and not _lib.same_elements(q, wide[:, 8:16])
+    assert not _lib.same_elements(q, wide.view(torch.int32)[:, :8])

@@ -126,3 +126,46 @@ def test_a_large_value_of_a_key_far_below_weighs_nothing(case, prefix, score):
         kv._k[0, page, at, 1], kv._v[0, page, at, 1] = kept
         _check(got, want, w)
     kv.check_errors()
+
+
+@pytest.mark.parametrize("kernel", [0, 1])
+def test_outputs_that_overlap_are_refused(kernel):
+    kv, g = _build(40, [10, 20], 2, 64, 16, BF, 1)
+    starts, shape = [8, 18], (2, 2, 4, 64)
+    batch = SharedPrefixBatch.from_lists(kv, 0, 40, [1, 2], starts, 2)
+    q = _query(g, 2, 2, 4, 64, BF)
+    exact = _exact(q, kv, 0, 40, starts)
+
+    def call(query, out):
+        return paged_attention_shared_prefix(query, kv, 0, batch, out=out, kernel=kernel)
+
+    flat = torch.zeros(4096, dtype=BF, device=DEV)
+    for stride in ((512, 128, 64, 1), (256, 256, 64, 1), (512, 256, 32, 1)):
+        with pytest.raises(ValueError, match="overlap"):
+            call(q, flat.as_strided(shape, stride))
+    n = q.numel()
+    for shift in (8, 64, 256, 512):  # the query shifted by a piece, a head, a chunk row, a sequence
+        query = flat[:n].view(shape)
+        query.copy_(q)
+        with pytest.raises(ValueError, match="overlap"):
+            call(query, flat[shift:shift + n].view(shape))
+        with pytest.raises(ValueError, match="overlap"):
+            call(flat[shift:shift + n].view(shape), query)
+    query = flat[:n].view(shape)
+    with pytest.raises(ValueError, match="overlap"):
+        call(query, flat.view(F32)[:n].view(shape))  # of another type at the same place
+    # the query itself, the memory behind it, and column blocks of the query's own rows
+    query.copy_(q)
+    _check(call(query, query), exact, BF if kernel == 0 else None)
+    query.copy_(q)
+    _check(call(query, flat[n:2 * n].view(shape)), exact, BF if kernel == 0 else None)
+    wide = torch.zeros((2, 2, 8 * 64), dtype=BF, device=DEV)
+    query, out = (wide[..., i * 256:(i + 1) * 256].view(shape) for i in range(2))
+    query.copy_(q)
+    for _ in range(2):
+        _check(call(query, out), exact, BF if kernel == 0 else None)
+    # a query that is copied first (its heads are not unit-stride) may lie where the output goes
+    turned = flat[:n].view(2, 2, 64, 4).transpose(2, 3)
+    turned.copy_(q)
+    _check(call(turned, flat[:n].view(shape)), exact, BF if kernel == 0 else None)
+    kv.check_errors()
