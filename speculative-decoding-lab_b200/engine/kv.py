@@ -35,7 +35,8 @@ from typing import Dict, List, Optional, Sequence
 import torch
 
 from . import _lib
-from .layer_ops import ROPE_PLANS_MAX, RopePlan, _check_heads, _check_out_rows, _has_head_rows, _rope_args, rope_key
+from .layer_ops import (ROPE_PLANS_MAX, RopePlan, _check_heads, _check_out_rows, _has_head_rows, _rope_args,
+                        check_apart, rope_key)
 from .utils import setup_logger
 
 logger = setup_logger(__name__)
@@ -370,7 +371,8 @@ class PagedKVCache:
         ``(T, num_kv_heads, head_dim)`` is rotated by ``positions`` and stored
         with ``vvecs`` at ``slots`` (int32, from ``reserve``); ``query``
         ``(T, heads, head_dim)``, when given, is rotated into ``query_out`` (a
-        new tensor by default, which may be ``query``) and returned.
+        new tensor by default; it may be ``query`` itself, and must not overlap
+        the inputs otherwise) and returned.
 
         ``table``, ``positions`` and ``sections`` are ``layer_ops.rope_axes``'s:
         positions are independent of the slots, so sequences that continue a
@@ -424,6 +426,7 @@ class PagedKVCache:
             _check_heads(query_out, "query_out", query.shape[0], query.shape[1], query.shape[2], query.dtype,
                          query.device)
             _check_out_rows(query_out, "query_out")
+            check_apart(plan, (("query_out", query_out),), (query, kvecs, vvecs))
             a.q_out_row_stride = query_out.stride(0)
         if not a.num_tokens:
             return query_out

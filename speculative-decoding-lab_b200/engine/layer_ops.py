@@ -167,6 +167,25 @@ def _check_out_rows(x: torch.Tensor, name: str) -> None:
         raise ValueError("{} needs rows of back-to-back heads that do not overlap".format(name))
 
 
+def check_apart(plan: "RopePlan", outs, inputs) -> None:
+    """Refuses outputs that share memory with each other or with an input;
+    ``outs`` are (name, output) in the order of their inputs, and an output may
+    be its own input itself.  The answer holds for the tensors' distances and row strides."""
+    base = inputs[0].data_ptr()
+    sig = tuple(t.data_ptr() - base for t in inputs) + tuple(
+        x for _, o in outs for x in (o.data_ptr() - base, o.stride(0)))
+    if sig == plan.apart:
+        return
+    for i, (name, o) in enumerate(outs):
+        for j, t in enumerate(inputs):
+            if not (j == i and _lib.same_elements(o, t)) and _lib.share_memory(o, t):
+                raise ValueError("{} must be its input itself or not overlap any".format(name))
+        for _, other in outs[:i]:
+            if _lib.share_memory(o, other):
+                raise ValueError("{} must not overlap another output".format(name))
+    plan.apart = sig
+
+
 def _empty_contiguous(x: torch.Tensor) -> torch.Tensor:
     return torch.empty_like(x, memory_format=torch.contiguous_format)
 
@@ -175,13 +194,14 @@ class RopePlan:
     """A checked argument struct of one combination of shapes, strides, types
     and thread; calls that hit it fill in the pointers."""
 
-    __slots__ = ("args", "ref", "device", "like_q", "like_k")
+    __slots__ = ("args", "ref", "device", "like_q", "like_k", "apart")
 
     def __init__(self, args: _lib.SdlRopeArgs, device: torch.device, q: Optional[torch.Tensor],
                  k: Optional[torch.Tensor]) -> None:
         self.args = args
         self.ref = ctypes.byref(args)
         self.device = device
+        self.apart = None  # distances of the tensors that check_apart has passed
         # new outputs (a contiguous input's layout is the default, which takes 0.3 us less)
         self.like_q, self.like_k = (
             torch.empty_like if x is None or x.is_contiguous() else _empty_contiguous for x in (q, k))
@@ -224,8 +244,9 @@ def rope_axes(q: torch.Tensor, k: Optional[torch.Tensor], table: torch.Tensor, p
     instead).  A pair whose position lies outside the table comes out NaN, the
     row's other pairs as usual.
 
-    ``out = (q_out, k_out)`` receives the result (rows of back-to-back heads;
-    they may be ``q`` and ``k`` themselves).
+    ``out = (q_out, k_out)`` receives the result (rows of back-to-back heads).
+    They may be ``q`` and ``k`` themselves, each its own input; outputs that
+    overlap an input otherwise, or each other, are refused.
     """
     key = rope_key(q, k, table, positions, sections)
     plan = _ROPE_PLANS.get(key)
@@ -265,6 +286,10 @@ def rope_axes(q: torch.Tensor, k: Optional[torch.Tensor], table: torch.Tensor, p
             if o is not None:
                 _check_heads(o, "out: " + name, x.shape[0], x.shape[1], x.shape[2], x.dtype, x.device)
                 _check_out_rows(o, "out: " + name)
+        if k is None:
+            check_apart(plan, (("out: q", qo),), (q,))
+        else:
+            check_apart(plan, (("out: q", qo), ("out: k", ko)), (q, k))
         a.q_out_row_stride = qo.stride(0)
         a.k_out_row_stride = 0 if ko is None else ko.stride(0)
     if not a.num_tokens or not (a.Hq or a.Hkv):

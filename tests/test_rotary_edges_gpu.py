@@ -106,3 +106,74 @@ def test_empty_calls_of_sliced_tensors(heads):
     assert turned.shape == (4, 0, 64)
     _check(other, k, table, pos, None)
     kv.check_errors()
+
+
+def test_outputs_that_overlap_inputs_or_each_other_are_refused():
+    T, hq, hkv, d = 6, 4, 2, 64
+    q, k, v, table, pos = _inputs(T, hq, hkv, d, torch.bfloat16, 1, 50, 1)
+    want = layer_ops.rope_axes(q, k, table, pos)
+    kv = _cache(hkv, d, torch.bfloat16, [T])
+    slots = kv.reserve([0], [0], [T])
+    flat = torch.zeros(8192, dtype=q.dtype, device=DEV)
+    nq, nk = q.numel(), k.numel()
+
+    def at(first, like):
+        return flat[first:first + like.numel()].view(like.shape)
+
+    fresh = at(0, q).copy_(q), at(nq, k).copy_(k)
+    free = at(4096, q), at(4096 + nq, k)
+    for shift in (8, 64, 256):
+        with pytest.raises(ValueError, match="overlap"):
+            layer_ops.rope_axes(fresh[0], fresh[1], table, pos, out=(at(shift, q), free[1]))
+        with pytest.raises(ValueError, match="overlap"):
+            layer_ops.rope_axes(fresh[0], fresh[1], table, pos, out=(free[0], at(nq + shift, k)))
+        with pytest.raises(ValueError, match="overlap"):
+            layer_ops.rope_axes(fresh[0], None, table, pos, out=(at(shift, q), None))
+        with pytest.raises(ValueError, match="overlap"):
+            layer_ops.rope_axes(fresh[0], fresh[1], table, pos, out=(free[0], at(4096 + shift, k)))
+        for inputs in ((fresh[0], k, v), (q, fresh[1], v), (q, k, fresh[1])):
+            out = at(shift, q) if inputs[0] is not q else at(nq + shift, q)
+            with pytest.raises(ValueError, match="overlap"):
+                kv.append_rotary(0, slots, inputs[1], inputs[2], table, pos, query=inputs[0], query_out=out)
+    # an output at the other input's place, and both at one place
+    same = at(0, k).copy_(k)
+    with pytest.raises(ValueError, match="overlap"):
+        layer_ops.rope_axes(same, k, table, pos, out=(free[1], same))
+    with pytest.raises(ValueError, match="overlap"):
+        layer_ops.rope_axes(k, k, table, pos, out=(free[1], free[1]))
+    for out in ((same, free[1]), (free[1], same), (same, same)):  # one tensor as q and k
+        with pytest.raises(ValueError, match="overlap"):
+            layer_ops.rope_axes(same, same, table, pos, out=out)
+    with pytest.raises(ValueError, match="overlap"):
+        kv.append_rotary(0, slots, same, v, table, pos, query=same, query_out=same)
+    # apart, in place, and in place in the columns of one projection, each twice
+    fresh[0].copy_(q), fresh[1].copy_(k)
+    for _ in range(2):
+        got = layer_ops.rope_axes(fresh[0], fresh[1], table, pos, out=free)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+        block = torch.cat((q.reshape(T, -1), k.reshape(T, -1), v.reshape(T, -1)), 1)
+        qb, kb = block[:, :hq * d].view(T, hq, d), block[:, hq * d:(hq + hkv) * d].view(T, hkv, d)
+        layer_ops.rope_axes(qb, kb, table, pos, out=(qb, kb))
+        assert torch.equal(qb, want[0]) and torch.equal(kb, want[1])
+        assert torch.equal(block[:, (hq + hkv) * d:], v.reshape(T, -1))
+    kv.check_errors()
+
+
+@pytest.mark.parametrize("dtype,d,rotary", [(torch.bfloat16, 64, 0), (torch.float32, 64, 32), (torch.float16, 10, 0)])
+def test_append_rotary_turns_the_query_in_place(dtype, d, rotary):
+    """``query_out`` the query itself: padding rows come out zero, the others
+    as in a new tensor."""
+    T, hq, hkv = 9, 6, 2
+    q, k, v, table, pos = _inputs(T, hq, hkv, d, dtype, 1, 50, 4, rotary)
+    kv = _cache(hkv, d, dtype, [T])
+    slots = kv.reserve([0], [0], [T]).clone()
+    slots[[2, 7]] = -1
+    want = kv.append_rotary(0, slots, k, v, table, pos, query=q)
+    pools = kv._k.clone(), kv._v.clone()
+    assert (want[[2, 7]] == 0).all()
+    kv._k.zero_(), kv._v.zero_()
+    for query in (q.clone(), torch.cat((q, q), 1)[:, :hq]):  # rows back to back, and strided
+        got = kv.append_rotary(0, slots, k, v, table, pos, query=query, query_out=query)
+        assert got is query and torch.equal(query, want)
+        assert torch.equal(kv._k, pools[0]) and torch.equal(kv._v, pools[1])
+    kv.check_errors()
