@@ -393,6 +393,8 @@ class PagedKVCache:
             dev, T = self.device, slots.numel()
             if slots.device != dev:
                 raise ValueError("slots must be on {}".format(dev))
+            if slots.is_floating_point() or slots.is_complex() or slots.dtype == torch.bool:
+                raise TypeError("slots must be int32, got {}".format(slots.dtype))
             _check_heads(kvecs, "kvecs", T, self.num_kv_heads, self.head_dim, self.dtype, dev)
             _check_heads(vvecs, "vvecs", T, self.num_kv_heads, self.head_dim, self.dtype, dev)
             if query is not None:
@@ -401,6 +403,8 @@ class PagedKVCache:
             if slots.dtype != torch.int32 or not slots.is_contiguous() or not _has_head_rows(kvecs) \
                     or not _has_head_rows(vvecs) or (query is not None and not _has_head_rows(query)) \
                     or (T > 1 and positions.stride(-1) != 1):
+                if slots.dtype == torch.int64:  # a slot past 32 bits stays outside the pool
+                    slots = slots.clamp(-1, 2 ** 31 - 1)
                 return self.append_rotary(layer, slots.to(torch.int32).contiguous(), kvecs.contiguous(),
                                           vvecs.contiguous(), table, positions.contiguous(), sections,
                                           None if query is None else query.contiguous(), query_out)

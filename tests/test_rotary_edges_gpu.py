@@ -177,3 +177,39 @@ def test_append_rotary_turns_the_query_in_place(dtype, d, rotary):
         assert got is query and torch.equal(query, want)
         assert torch.equal(kv._k, pools[0]) and torch.equal(kv._v, pools[1])
     kv.check_errors()
+
+
+def test_wide_slots_do_not_wrap():
+    """64-bit slots are those of 32 bits; one past 32 bits lies outside the
+    pool, as any other too large, and is not another row's."""
+    T = 5
+    q, k, v, table, pos = _inputs(T, 4, 2, 64, torch.bfloat16, 1, 50, 1)
+    kv = _cache(2, 64, torch.bfloat16, [T])
+    slots = kv.reserve([0], [0], [T])
+    kv.append_rotary(0, slots, k, v, table, pos)
+    want = kv._k.clone(), kv._v.clone()
+    kv._k.zero_(), kv._v.zero_()
+    kv.append_rotary(0, slots.long(), k, v, table, pos)
+    assert torch.equal(kv._k, want[0]) and torch.equal(kv._v, want[1])
+    kv.check_errors()
+    for far in (2 ** 32, 2 ** 32 + int(slots[1]), 2 ** 31, 2 ** 62):
+        kv._k.zero_(), kv._v.zero_()
+        wide = slots.long()
+        wide[3] = far
+        kv.append_rotary(0, wide, k, v, table, pos)
+        with pytest.raises(RuntimeError, match="0x10"):
+            kv.check_errors()
+        live = [0, 1, 2, 4]
+        at = slots[live].long()
+        assert torch.equal(kv._v[0].view(-1, 2, 64)[at], v[live])
+        kv._v[0].view(-1, 2, 64)[at] = 0
+        assert (kv._v == 0).all()
+    kv._v.zero_()
+    wide = slots.long()
+    wide[3] = -2 ** 33 + int(slots[0])  # negative: padding
+    turned = kv.append_rotary(0, wide, k, v, table, pos, query=q)
+    assert (turned[3] == 0).all()
+    kv.check_errors()
+    for dtype in (torch.float32, torch.bool, torch.bfloat16):
+        with pytest.raises(TypeError, match="slots"):
+            kv.append_rotary(0, slots.to(dtype), k, v, table, pos)
