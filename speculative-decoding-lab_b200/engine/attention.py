@@ -552,6 +552,16 @@ def _prefix_args(q, kv, layer, batch, out, kernel, prefix_split, own_split) -> _
     return x
 
 
+def _prefix_query(q, kv) -> torch.Tensor:
+    """``q``, or a copy of the type and layout that the kernels take (tensor
+    cores: 16-byte pieces)."""
+    q2 = q if q.dtype == kv.dtype else q.to(kv.dtype)
+    if q2.stride(3) != 1 or (kv.tensor_maps()[0] is not None and (q2.data_ptr() | 2 * q2.stride(0) | 2 * q2.stride(1)
+                                                                  | 2 * q2.stride(2)) % 16):
+        q2 = q2.clone(memory_format=torch.contiguous_format)
+    return q2
+
+
 PREFIX_KERNEL_NAMES = (None, "generic", "mma", "tcgen05")
 
 
@@ -559,6 +569,7 @@ def prefix_attention_kernel(q: torch.Tensor, kv: PagedKVCache, batch: SharedPref
     """Which kernel ``paged_attention_shared_prefix`` runs for these
     arguments: "generic" (CUDA cores), "mma" (mma.sync for prefix and own
     keys) or "tcgen05" (the prefix on the 5th-generation tensor cores)."""
+    q = _prefix_query(q, kv)
     x = _prefix_args(q, kv, 0, batch, q, 0, 0, 0)
     n = _lib.load().sdl_prefix_attention_kernel(ctypes.byref(x))
     if n < 0:
@@ -604,11 +615,7 @@ def paged_attention_shared_prefix(
     plan = batch._plans.get(key)
     if plan is None or plan.kv() is not kv or plan.table is not kv._table:
         _check_prefix_call(q, kv, batch, out, out_dtype)
-        # dtype and layout the kernels take (tensor cores: 16-byte pieces of q)
-        q2 = q if q.dtype == kv.dtype else q.to(kv.dtype)
-        if q2.stride(3) != 1 or (kv.tensor_maps()[0] is not None and (q2.data_ptr() | 2 * q2.stride(0) | 2 * q2.stride(1)
-                                                                      | 2 * q2.stride(2)) % 16):
-            q2 = q2.clone(memory_format=torch.contiguous_format)
+        q2 = _prefix_query(q, kv)
         if q2 is not q:
             if out is None:
                 out_dtype = out_dtype or kv.dtype

@@ -8,7 +8,7 @@ from __future__ import annotations
 import pytest
 import torch
 
-from engine.attention import SharedPrefixBatch, paged_attention_shared_prefix
+from engine.attention import SharedPrefixBatch, paged_attention_shared_prefix, prefix_attention_kernel
 from test_shared_prefix_gpu import BF, DEV, F32, HF, PLANTS, _build, _check, _exact, _planted, _query
 
 pytestmark = pytest.mark.gpu
@@ -168,4 +168,24 @@ def test_outputs_that_overlap_are_refused(kernel):
     turned = flat[:n].view(2, 2, 64, 4).transpose(2, 3)
     turned.copy_(q)
     _check(call(turned, flat[:n].view(shape)), exact, BF if kernel == 0 else None)
+    kv.check_errors()
+
+
+def test_the_named_kernel_is_the_one_that_runs():
+    """For queries that the call copies first: of another type, off 16-byte
+    boundaries, with strided dims."""
+    P, owns, chunk = 300, [40, 30, 20, 9], 5
+    kv, g = _build(P, owns, 2, 128, 16, BF, 8)
+    starts = [n - chunk for n in owns]
+    batch = SharedPrefixBatch.from_lists(kv, 0, P, [1, 2, 3, 4], starts, chunk)
+    q = _query(g, 4, chunk, 12, 128, BF)
+    want = paged_attention_shared_prefix(q, kv, 0, batch)
+    assert prefix_attention_kernel(q, kv, batch) == "tcgen05"
+    assert torch.equal(want, paged_attention_shared_prefix(q, kv, 0, batch, kernel=3))
+    odd = torch.zeros(q.numel() + 1, dtype=BF, device=DEV)[1:].view(q.shape).copy_(q)
+    turned = q.transpose(2, 3).contiguous().transpose(2, 3)
+    rows = torch.zeros((4, chunk, 12, 130), dtype=BF, device=DEV)[..., :128].copy_(q)
+    for same in (q.float(), odd, turned, rows):
+        assert prefix_attention_kernel(same, kv, batch) == "tcgen05"
+        assert torch.equal(paged_attention_shared_prefix(same, kv, 0, batch), want)
     kv.check_errors()
