@@ -457,19 +457,25 @@ class SharedPrefixBatch(AttnBatch):
 
     def __init__(self, prefix_id: int, prefix_len: int, rows: torch.Tensor, starts: torch.Tensor, max_limit: int,
                  valid_rows: Optional[torch.Tensor] = None, key_count: int = 0) -> None:
-        for name, t in (("rows", rows), ("starts", starts), ("valid_rows", valid_rows)):
-            if t is None and name == "valid_rows":
-                continue
-            _lib.require_cuda(t, name)
-            if t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous() or t.numel() != rows.numel() \
-                    or t.device != rows.device:
-                raise ValueError("{} must be contiguous int32 with one entry per sequence".format(name))
         super().__init__(rows, starts, max_limit, valid_rows, key_count)
+        self.check_tensors()
         self.prefix_id = int(prefix_id)
         self.prefix_len = int(prefix_len)
         if self.prefix_id < 0 or self.prefix_len < 0:
             raise ValueError("prefix_id and prefix_len must not be negative")
         self._plans = {}
+
+    def check_tensors(self) -> None:
+        """Refuses rows, starts or valid_rows that the kernels cannot read, as
+        given or as set since."""
+        for name in ("rows", "starts", "valid_rows"):
+            t = getattr(self, name)
+            if t is None and name == "valid_rows":
+                continue
+            _lib.require_cuda(t, name)
+            if t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous() or t.numel() != self.rows.numel() \
+                    or t.device != self.rows.device:
+                raise ValueError("{} must be contiguous int32 with one entry per sequence".format(name))
 
     @classmethod
     def from_lists(cls, kv: PagedKVCache, prefix_id: int, prefix_len: int, seq_ids: Sequence[int],
@@ -526,6 +532,7 @@ def _check_prefix_call(q, kv, batch, out, out_dtype) -> None:
     _lib.require_cuda(q, "query")
     if q.dim() != 4 or q.shape[3] != kv.head_dim:
         raise ValueError("query must be (B, chunk, Hq, {}), got {}".format(kv.head_dim, tuple(q.shape)))
+    batch.check_tensors()
     dev = kv.device
     if q.device != dev or batch.rows.device != dev:
         raise ValueError("query and batch must be on the cache's device {}".format(dev))

@@ -189,3 +189,25 @@ def test_the_named_kernel_is_the_one_that_runs():
         assert prefix_attention_kernel(same, kv, batch) == "tcgen05"
         assert torch.equal(paged_attention_shared_prefix(same, kv, 0, batch), want)
     kv.check_errors()
+
+
+def test_tensors_set_on_a_batch_in_use_are_checked():
+    kv, g = _build(60, [40, 30], 2, 64, 16, BF, 3)
+    q = _query(g, 2, 1, 4, 64, BF)
+    batch = SharedPrefixBatch.from_lists(kv, 0, 60, [1, 2], [39, 29], 1)
+    exact = _exact(q, kv, 0, 60, [39, 29])
+    _check(paged_attention_shared_prefix(q, kv, 0, batch), exact, BF)
+    for name, value in (("starts", torch.tensor([39, 29], device=DEV)), ("starts", _i32(39)), ("rows", _i32(1)),
+                        ("rows", _i32(1, 7, 2, 7)[::2]), ("valid_rows", _i32(1, 1, 1)),
+                        ("valid_rows", torch.ones(2, device=DEV)), ("starts", _i32(39, 29)[:, None])):
+        kept = getattr(batch, name)
+        setattr(batch, name, value)
+        with pytest.raises(ValueError, match="int32"):
+            paged_attention_shared_prefix(q, kv, 0, batch)
+        setattr(batch, name, kept)
+    batch.starts = torch.tensor([39, 29], dtype=torch.int32)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        paged_attention_shared_prefix(q, kv, 0, batch)
+    batch.starts = _i32(39, 29)
+    _check(paged_attention_shared_prefix(q, kv, 0, batch), exact, BF)
+    kv.check_errors()
