@@ -19,6 +19,7 @@
 #include "sdl_common.cuh"
 
 #include <algorithm>
+#include <climits>
 
 namespace {
 
@@ -323,6 +324,7 @@ int run_rope(const sdl_rope_args* a, bool append, void* stream, const char* what
         return bad(SDL_ERR_UNSUPPORTED, "unsupported dtype");
     if (a->num_tokens < 0 || a->Hq < 0 || a->Hkv < 0 || a->head_dim < 1 || a->head_dim > 1024)
         return bad(SDL_ERR_INVALID, "bad shape arguments");
+    if (a->num_tokens > INT_MAX - 64) return bad(SDL_ERR_UNSUPPORTED, "too many rows");  // of blocks of up to 64
     if (a->num_tokens == 0) return SDL_OK;
     if (!a->table || a->table_rows < 1 || a->rotary < 2 || a->rotary % 2 || a->rotary > a->head_dim)
         return bad(SDL_ERR_INVALID, "table needs rows of cos and sin over an even rotary width of at most head_dim");

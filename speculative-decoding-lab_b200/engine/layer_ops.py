@@ -119,6 +119,8 @@ def _rope_args(table: torch.Tensor, positions: torch.Tensor, sections: Optional[
     rotary = table.shape[2]
     if rotary < 2 or rotary % 2 or rotary > head_dim or table.shape[0] < 1:
         raise ValueError("table: rotary width {} must be even and at most head_dim {}".format(rotary, head_dim))
+    if tokens > ROPE_TOKENS_MAX:
+        raise ValueError("{} rows in one call, of {} at most".format(tokens, ROPE_TOKENS_MAX))
     nd = positions.dim()
     if nd not in (1, 2) or positions.shape[-1] != tokens:
         raise ValueError("positions must be (tokens,) or (axes, tokens) for {} tokens, got {}".format(
@@ -218,6 +220,7 @@ class RopePlan:
 
 _ROPE_PLANS = {}
 ROPE_PLANS_MAX = 256
+ROPE_TOKENS_MAX = 2 ** 31 - 65  # rows are counted in 32 bits, a block's 64 past the last included
 
 
 def rope_key(q, k, table, positions, sections):

@@ -72,3 +72,22 @@ def test_shared_memory_is_found_byte_by_byte():
     q = wide[:, :8]
     assert _lib.same_elements(q, q.view(50, 8)) and not _lib.same_elements(q, wide[:, 8:16])
     assert not _lib.same_elements(q, wide.view(torch.int32)[:, :8])
+
+
+def test_rows_past_32_bits_are_refused():
+    """Counts are 32 bits wide below: 2^31 + 1 rows are not one row."""
+    import ctypes
+
+    from engine import _lib, layer_ops
+    from test_shared_prefix_cpu import _rope
+
+    table = torch.empty((10, 2, 64), device="meta")
+    for tokens in (2 ** 31 - 64, 2 ** 31, 2 ** 32 + 1):
+        pos = torch.empty(tokens, dtype=torch.int64, device="meta")
+        with pytest.raises(ValueError, match="rows"):
+            layer_ops._rope_args(table, pos, None, tokens, 64, table.device)
+    pos = torch.empty(2 ** 31 - 65, dtype=torch.int64, device="meta")
+    assert layer_ops._rope_args(table, pos, None, 2 ** 31 - 65, 64, table.device).num_tokens == 2 ** 31 - 65
+    for fn in ("sdl_rope_axes", "sdl_kv_append_rotary"):
+        for tokens in (2 ** 31 - 64, 2 ** 31 - 1):
+            assert getattr(_lib.load(), fn)(ctypes.byref(_rope(num_tokens=tokens)), None) == 2  # SDL_ERR_UNSUPPORTED
