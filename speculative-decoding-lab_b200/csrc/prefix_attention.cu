@@ -1790,6 +1790,7 @@ bool tensor_cores_apply(const sdl_attn_args* a) {
 }
 
 constexpr int kSms = 148;
+constexpr int64_t kOwnPartials = int64_t(1) << 30;  // bytes of partials from which own ranges are not cut further
 constexpr int kMaxSmem = 225 * 1024;  // dynamic shared memory of a block beside 2 KB of static
 
 // Keys per prefix range of the tcgen05 kernel: the number of ranges with the
@@ -1916,6 +1917,13 @@ int make_plan(const sdl_prefix_args* x, Plan& pl) {
                              kStageKeys);
         }
     }
+    // Own ranges are bounded above, however many rows there are; where their
+    // partials would pass 1 GiB the rows alone fill the SMs many times over, and
+    // the ranges grow instead (256 x 128 rows of 32 heads with up to 32768 own
+    // keys: 0.5 GiB in one range, 17 in ranges of 1024).
+    const int64_t range = (int64_t)p.F * p.Hkv * (p.hd + 2) * (int64_t)sizeof(float);
+    if (cdiv(span, p.mpk) * range > kOwnPartials)
+        p.mpk = round_up(cdiv(span, std::max<int64_t>(1, kOwnPartials / range)), kStageKeys);
     if (x->prefix_split) p.ppk = round_up(std::min(x->prefix_split, 1 << 29), page);
     if (x->own_split) p.mpk = round_up(std::min(x->own_split, 1 << 29), page);
     p.nsp = cdiv(x->prefix_len, p.ppk);

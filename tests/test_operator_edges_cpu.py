@@ -91,3 +91,37 @@ def test_rows_past_32_bits_are_refused():
     for fn in ("sdl_rope_axes", "sdl_kv_append_rotary"):
         for tokens in (2 ** 31 - 64, 2 ** 31 - 1):
             assert getattr(_lib.load(), fn)(ctypes.byref(_rope(num_tokens=tokens)), None) == 2  # SDL_ERR_UNSUPPORTED
+
+
+@pytest.mark.parametrize("kw", [
+    dict(B=256, chunk=128, Hq=32, Hkv=8, max_limit=32768),
+    dict(B=256, chunk=128, Hq=32, Hkv=8, max_limit=32768, prefix_len=0),
+    dict(B=512, chunk=1, Hq=64, Hkv=8, max_limit=40000, key_count=512 * 100),
+    dict(B=512, chunk=64, Hq=32, Hkv=8, max_limit=32768, out_dtype=0),          # mma.sync
+    dict(B=2000, chunk=64, Hq=4, Hkv=2, head_dim=64, max_limit=32768, dtype=0, out_dtype=0, key_count=2000 * 64),
+], ids=str)
+def test_the_workspace_of_many_rows_is_bounded(kw):
+    """Own ranges take 1 GiB of partials, or one range of all keys; prefix
+    ranges one for rows as many as these, or a few."""
+    import ctypes
+
+    from engine import _lib
+    from test_shared_prefix_cpu import _attn
+
+    x = _attn(**dict(dict(width=4096, capacity=100000), **kw))
+    need = _lib.load().sdl_prefix_attention_workspace_bytes(ctypes.byref(x))
+    a = x.attn
+    one = a.B * a.chunk * a.Hq * (a.head_dim + 2) * 4
+    assert 0 < need <= max(one, 2 ** 30) + 4 * one, need / one
+
+
+def test_the_workspace_of_ordinary_calls_is_as_it_was():
+    """Ranges of 512 own keys (mma.sync, 64 decode rows) where they are few."""
+    import ctypes
+
+    from engine import _lib
+    from test_shared_prefix_cpu import _attn
+
+    x = _attn(B=64, max_limit=32768, width=4096, prefix_len=0, kernel=2)
+    need = _lib.load().sdl_prefix_attention_workspace_bytes(ctypes.byref(x))
+    assert need == 64 * 12 * 64 * (128 + 2) * 4

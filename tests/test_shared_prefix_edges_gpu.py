@@ -211,3 +211,20 @@ def test_tensors_set_on_a_batch_in_use_are_checked():
     batch.starts = _i32(39, 29)
     _check(paged_attention_shared_prefix(q, kv, 0, batch), exact, BF)
     kv.check_errors()
+
+
+@pytest.mark.parametrize("kernel", [0, 2])
+def test_own_ranges_that_grow_for_many_rows(kernel):
+    """A bound whose partials would pass the workspace's: 32768 rows of up to
+    40000 own keys, of which one sequence has many."""
+    B, P, hq, hkv, d = 512, 70, 64, 8, 128
+    owns = [1 + i % 90 for i in range(B)]
+    owns[300] = 20011
+    kv, g = _build(P, owns, hkv, d, 16, BF, 6, extra=2600)
+    q = _query(g, B, 1, hq, d, BF)
+    starts = [n - 1 for n in owns]
+    rows = torch.arange(1, B + 1, dtype=torch.int32, device=DEV)
+    batch = SharedPrefixBatch(0, P, rows, _i32(*starts), 40000)
+    got = paged_attention_shared_prefix(q, kv, 0, batch, kernel=kernel)
+    _check(got, _exact(q, kv, 0, P, starts), BF)
+    kv.check_errors()
