@@ -68,9 +68,9 @@ SDL_DEV int pfx_nvalid(const PfxParams& p, int b) {
 // Own keys that row j of sequence b attends: starts[b] + j + 1, within [0,
 // max_limit].  `over` where the bound cuts some off (the merge reports it).
 SDL_DEV int pfx_limit(const PfxParams& p, int b, int j, bool& over) {
-    const int64_t n = (int64_t)p.starts[b] + j + 1;
-    over = n > p.max_limit;
-    return (int)max((int64_t)0, min(n, (int64_t)p.max_limit));
+    const int start = p.starts[b];
+    over = start > p.max_limit - 1 - j;  // so written, nothing overflows
+    return over ? p.max_limit : max(0, start + j + 1);
 }
 
 // One item: flat rows [f0, f1) of kv head g against keys [k0, k1) of the
@@ -1629,11 +1629,11 @@ __global__ void __launch_bounds__(kMergeWarps * 32) prefix_merge_kernel(const __
     if (p.nsp + p.nsm == 0) pdl_wait();  // no items: the call's first kernel
     const FlatRow r = pfx_row(p, f, g);
     const int ns = in && r.valid ? p.nsp + min(p.nsm, (r.limit + p.mpk - 1) / p.mpk) : 0;  // nsm 0 with own_direct
+    if (in && r.valid && r.over && lane % LANES == 0) sdl_raise(p.err, SDL_DEVERR_BAD_INDEX);
     // the row's metadata was read under the items' tail: whatever wrote it was
     // complete before they ran; the partials only now
     pdl_wait();
     pdl_launch_dependents();
-    if (in && r.valid && r.over && lane % LANES == 0) sdl_raise(p.err, SDL_DEVERR_BAD_INDEX);
     if (WARPS == 1 && !(in && r.valid)) return;
     const int d0 = (lane % LANES) * 4;
     const float* op = p.o_part + w * p.nslot * HD + d0;
