@@ -343,14 +343,15 @@ int sdl_prefill_chunk(const sdl_attn_args* args, void* stream);
  * starts[b] + j.  It attends, in one softmax, positions [0, prefix_len) of
  * block-table row `prefix_row` and own positions [0, starts[b] + j]; starts
  * may be negative (a row without own keys), and a row with no key at all
- * comes out zero.  Rows j >= valid_rows[b] are not written.  `max_limit`
- * bounds starts[b] + chunk: a row attends own positions below it only, and a
- * written row that it cuts off is reported (SDL_DEVERR_BAD_INDEX).  k_new / rope_cos / dense K/V are refused, and the
- * plan fields of `attn` (pages_per_split .. mma_layout, overlap_layers) are
- * not read, except key_count: 0, or the host's sum of starts[b] + chunk.
- * Pool rows that a query row does not attend may hold any value, NaN
- * included.  `scale` is positive; at most 2^30 - 1 keys and query rows.  `out`
- * may be `q` itself. */
+ * comes out zero, as does one all of whose scores are -inf.  Rows
+ * j >= valid_rows[b] are not written.  `max_limit` bounds starts[b] + chunk: a
+ * row attends own positions below it only, and a written row that it cuts off
+ * is reported (SDL_DEVERR_BAD_INDEX).  k_new / rope_cos / dense K/V are
+ * refused, and the plan fields of `attn` (pages_per_split .. mma_layout,
+ * overlap_layers) are not read, except key_count: 0, or the host's sum of
+ * starts[b] + chunk.  Pool rows that a query row does not attend may hold any
+ * value, NaN included.  `scale` is positive; at most 2^30 - 1 keys and query
+ * rows.  `out` may be `q` itself, and must not overlap it otherwise. */
 typedef struct sdl_prefix_args {
     sdl_attn_args attn;
     int32_t table_rows;    /* rows of block_table; `rows` outside are
@@ -559,7 +560,8 @@ typedef struct sdl_rope_args {
     int32_t num_layers, layer, capacity, block_size;
 } sdl_rope_args;
 
-/* q_out and k_out receive the turned rows (strides in elements). */
+/* q_out and k_out receive the turned rows (strides in elements).  They may be
+ * q and k in place, and overlap no input otherwise, nor each other. */
 int sdl_rope_axes(const sdl_rope_args* args, void* stream);
 
 /* Stores the turned k row and the v row of token t at slots[t] of layer

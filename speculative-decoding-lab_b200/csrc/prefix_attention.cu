@@ -14,6 +14,10 @@
 // Items write fp32 partials [g][f][slot], prefix ranges first, then own
 // ranges; prefix_merge_kernel joins them (fixed order: results do not depend
 // on scheduling).
+//
+// Times below are of whole calls in a captured graph of 30, over three sets of
+// inputs in turn; those of 50 us and more move by up to 5 % with the clock that
+// the power limit leaves.  A call through Python takes 10 to 13 us at least.
 #include "sdl_common.cuh"
 
 #include <cuda.h>
@@ -339,9 +343,9 @@ SDL_DEV uint64_t add_f32x2(uint64_t a, uint64_t b) {
 // are packed in pairs (fma.rn.f32x2; of dims in both products), fp32 tiles
 // arrive by cp.async under the softmax and the other product.  Bound by the 12
 // reads of 16 bytes for 128 products (shared memory 71 % busy, issue slots 47 %):
-// 8192 rows x 2 heads behind 4096 keys, d 64, 608 us (29 TFLOP/s; 628 with plain
-// loads, 657 without the pairs either); 2304 x 2 behind 2000, d 128, 305 us
-// (351, 367).  Eight rows a thread read less and hide less (two blocks per SM):
+// 8192 rows x 2 heads behind 4096 + 1..300 keys, d 64, 621 us (29 TFLOP/s); 2304
+// x 2 behind 2000 + 1..300, d 128, 340 us (15).  Plain loads cost 3 % and 15 %,
+// products without pairs another 5 %.  Eight rows a thread read less and hide less (two blocks per SM):
 // no gain.
 constexpr int kWideRows = 64, kWideKeys = 64, kWidePitch = kWideKeys + 4;
 
@@ -668,8 +672,8 @@ struct MmaCfg {
     // d 128: two CTAs per SM, 96 KB rings; 256 threads launch with 128 registers
     // each, of which the consumer warpgroup takes 200 and the producers keep 56
     // (128 * 200 + 128 * 56 = 256 * 128).  d 64: three CTAs, 64 KB rings, 80
-    // registers shared as 128 and 32 (256 decode rows behind 2051 keys: 23.0
-    // us, 24.5 with two CTAs; 200 rows of 8 heads: 27.7 and 31.9).
+    // registers shared as 128 and 32 (256 decode rows behind 2051 keys: 23.9
+    // us, 26.2 with two CTAs; 200 rows of 8 kv heads: 47.4 and 56.2).
     static constexpr int kCtas = HD == 128 ? 2 : 3;
     static constexpr int kStages = HD == 128 ? 3 : 4;
     static constexpr int kRegs = HD == 128 ? 200 : 128, kHelpRegs = HD == 128 ? 56 : 32;
@@ -1026,8 +1030,8 @@ prefix_mma_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant
 // four producers 4200, elected issue and part of the exponentials on the FMA
 // pipe 3200.  64-key S products read 6 KB of operands per 32 cycles of MMA, 48
 // at the shared memory's 128 bytes a cycle (2560 a step): the overlap pays it.
-// 256 x 6 rows behind 16384 keys run at 1.4 PFLOP/s, of 1.7 for a large matrix
-// product.
+// 256 x 6 rows of 12 heads behind 16384 keys alone take 150 us with the merge:
+// 1.03 PFLOP/s (a large matrix product: 1.70 in a burst, 1.42 sustained).
 // TMEM: score buffers (tile t, i & 1) of 64 columns, then O_t, 128 apart.
 constexpr int kURows = 128;                 // rows of one tile (MMA M)
 constexpr int kUKeys = 64;                  // keys per step
@@ -1393,8 +1397,8 @@ prefix_umma_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constan
                     unpack_f32x2(fma_f32x2(pack_f32x2(s[2 * e], s[2 * e + 1]), scale2, base2), p0, p1);
                     // one pair of four on the FMA pipe, as the special function
                     // unit needs 8 cycles for a warp's value (16 x 96 rows
-                    // behind 6000 keys: none 102 us, 1/8 99, 1/4 94, 3/8 96,
-                    // 1/2 101)
+                    // behind 6000 keys: none 92 us, 1/8 93, 1/4 90, 3/8 92,
+                    // 1/2 95; 256 x 6 behind 16384: 188, 187, 188, 193, 195)
                     if ((e & 3) == 1) {
                         ex2_poly2(p0, p1);
                     } else {
@@ -1471,8 +1475,9 @@ prefix_umma_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constan
 // softmax.  Where no sequence has more than a page of own keys (own_direct), it
 // attends them here, four keys at a time, in place of a launch whose items
 // would last longer than their keys (105 decode rows of 32 / 8 heads with 2 to 4
-// own keys behind 2707: 21.5 us, 25.3 with 840 own items).  WARPS = 1: a warp takes whole rows; WARPS = 4 (many slots, few
-// rows): a block's warps share a row's slots and join in shared memory.
+// own keys behind 2707: 21.6 us, 25.8 with 840 own items).  WARPS = 1: a warp
+// takes whole rows; WARPS = 4 (many slots, few rows): a block's warps share a
+// row's slots and join in shared memory.
 constexpr int kMergeWarps = 4;
 constexpr int kMergeMany = 12;  // slots from which a row takes four warps
 
@@ -1799,9 +1804,9 @@ constexpr int kMaxSmem = 225 * 1024;  // dynamic shared memory of a block beside
 // + 12.5 per key, an own item 4000 + 12 per key.  Prefix items run in waves;
 // own items fill what they leave, and begin late where the slots do not hold
 // all.  Every range writes, and the merge reads, a partial of `elems` fp32
-// values in all, at about 6 bytes per ps and 50 ns of latency.  (Fitted to sweeps; 64 decode rows
-// behind 8192 keys with up to 1024 own: 512 keys 20.3 us, 384 25.2, 1024 22.1;
-// 16 x 96 rows behind 6000: 2048 83 us, 1024 108, 6000 93.)
+// values in all, at about 6 bytes per ps and 50 ns of latency.  (Fitted to sweeps; 64
+// decode rows behind 8192 keys with up to 1024 own: 512 keys 20.9 us, 384 24.8,
+// 1024 24.1; 16 x 96 rows behind 6000: 2048 91 us, 1024 113, 6000 100.)
 int umma_prefix_split(int prefix, int64_t tiles, bool big, int64_t elems, int64_t own_items, int64_t own_keys) {
     const int64_t slots = big ? kSms : 2 * kSms;
     const int64_t own = big ? (own_items + 1) / 2 : own_items, t_own = own_items ? 4000 + 12 * own_keys : 0;
@@ -1826,10 +1831,10 @@ int umma_prefix_split(int prefix, int64_t tiles, bool big, int64_t elems, int64_
 
 // Whether the prefix goes to the tcgen05 kernel, a launch more than mma.sync
 // alone: wherever the rows are more than one mma.sync operand holds (24 rows x
-// 2 kv heads, d 128, behind 256 keys: 13.3 us with mma.sync, 9.3 with tcgen05;
-// 28 x 2, d 64: 8.5 and 7.9), and fewer rows only over a long prefix in many
-// heads (4 x 8, d 128, behind 4096 keys: 9.7 and 13.4; behind 16384: 22.6 and
-// 19.3; at d 64 the two meet there).
+// 2 kv heads, d 128, behind 256 keys: 10.2 us with mma.sync, 8.8 with tcgen05;
+// 28 x 2, d 64: 7.5 and 6.7), and fewer rows only over a long prefix in many
+// heads (4 x 8, d 128, behind 4096 keys: 8.7 and 10.0; behind 16384: 22.6 and
+// 19.0; at d 64, 15.1 and 15.6).
 bool tcgen05_pays(const sdl_prefix_args* x) {
     const sdl_attn_args* a = &x->attn;
     const int64_t rows = (int64_t)a->B * a->chunk * (a->Hq / a->Hkv), keys = (int64_t)x->prefix_len * a->Hkv;
@@ -1869,9 +1874,9 @@ int make_plan(const sdl_prefix_args* x, Plan& pl) {
     // Prefix items of 256 rows share their K and V, which pays where they fill
     // the SMs at head_dim 128; otherwise items of 128 rows at two CTAs per SM mix
     // with the own items on every SM (us with 128 / 256 rows: 32 x 6 verify
-    // rows, 10 items of 256, 23.6 / 27.7; 160 x 6, 46 items, 59.3 / 58.8; 256 x 6
-    // behind 16384 keys, 72 items, 179 / 165; at d 64, 300 x 6, 100 items, 62.3 /
-    // 65.9).
+    // rows, 10 items of 256, 19.2 / 21.8; 160 x 6, 46 items, 49.7 / 49.6; 256 x 6
+    // behind 16384 keys, 72 items, 194 / 188; at d 64, 300 x 6, 100 items, 71.3 /
+    // 74.7).
     if (pl.kernel == 3) {
         pl.ptile = p.hd == 128 && (int64_t)cdiv(p.F, 2 * kURows) * p.Hkv >= 64 ? 2 * kURows : kURows;
     } else {
@@ -1887,9 +1892,10 @@ int make_plan(const sdl_prefix_args* x, Plan& pl) {
     const int64_t mean = a->key_count > 0 && a->B > 0 ? std::min<int64_t>(span, a->key_count / a->B + 1) : span;
     const int page = pl.kernel == 1 ? 1 : kPage;
     // At most a page of own keys each: in the merge, where own items would fill
-    // more than a wave and the rows are not many (us in the merge / as items: 500
-    // decode rows x 12 heads 17.6 / 24.1, 1600 x 8 heads 12.2 / 19.1; 32 x 8 rows
-    // x 12 heads, 64 items, 11.9 / 9.8; 60 x 8 x 32, 480 items, 34.3 / 30.9).
+    // more than a wave and the rows are not many (us in the merge / as items, behind
+    // 2000 keys: 500 decode rows x 12 heads 24.8 / 33.5; 32 x 8 rows x 12 heads,
+    // 64 items, 20.3 / 17.4; 60 x 8 x 32, 480 items, 46.7 / 43.3.  The row limit
+    // is too low for decode: 1600 rows x 8 heads, d 64, 30.9 / 81.5).
     const bool own_direct = pl.kernel >= 2 && span > 0 && span <= kPage && !x->own_split && mtiles > 2 * kSms &&
                             (int64_t)p.F * p.Hkv <= 8192;
     if (pl.kernel == 1) {
@@ -1898,9 +1904,10 @@ int make_plan(const sdl_prefix_args* x, Plan& pl) {
         p.ppk = p.mpk = round_up(std::max<int64_t>(64, std::min<int64_t>(std::max(x->prefix_len, span), keys)), kWideKeys);
     } else {
         // own keys: one item per SM where sequences are few, in bounded ranges.
-        // mma.sync (64 decode rows of 1..1024 own keys: 512 14.6 us, 256 17.3,
-        // 1024 19.7); tcgen05 (32 x 6 rows of 1..512: 256 13.4 us, 128 14.6,
-        // 512 15.5; 256 x 6 of 64..1024: 1024 52.8, 512 60.2, 256 77.7)
+        // mma.sync (64 decode rows of 1..1024 own keys behind 8192: 512 20.6 us,
+        // 256 23.9, 1024 25.6); tcgen05 (32 x 6 rows of 1..512 behind 4001: 256
+        // 19.2 us, 128 24.1, 512 20.9; 256 x 6 of 64..1024 behind 16384: 1024 190,
+        // 512 193, 256 207)
         const int64_t least = pl.own_umma ? 256 : 128, most = pl.own_umma ? 1024 : 512;
         p.mpk = round_up(std::max(least, std::min(most, mtiles * mean / kSms)), kStageKeys);
         const int64_t keys = ptiles * x->prefix_len + mtiles * mean;
@@ -1911,8 +1918,8 @@ int make_plan(const sdl_prefix_args* x, Plan& pl) {
                                       own, std::min<int64_t>(mean, p.mpk));
         } else {
             // two waves of two CTAs per SM, at least three or four stages (2
-            // rows x 2 heads behind 2000 keys: 192 8.3 us, 256 9.1, 512 12.2;
-            // behind 8000: 256 10.5, 192 11.2, 128 11.5)
+            // rows x 2 heads behind 2000 keys: 192 6.6 us, 256 7.2, 512 10.4;
+            // behind 8000: 256 8.4, 192 7.7, 128 7.5)
             p.ppk = round_up(std::max<int64_t>((x->prefix_len <= 4096 ? 3 : 4) * kStageKeys, std::min<int64_t>(x->prefix_len, keys / (kSms * 4))),
                              kStageKeys);
         }
@@ -2058,7 +2065,8 @@ int launch_tensor(const Plan& pl, const CUtensorMap& mk, const CUtensorMap& mv, 
 int launch_merge(const Plan& pl, cudaStream_t st) {
     const PfxParams& p = pl.p;
     const int64_t rows = (int64_t)p.F * p.Hkv;
-    // few rows spread over more warps earlier (32 x 6 verify rows, 7 slots: 20.3 us in all, 23.5)
+    // few rows spread over more warps earlier (32 x 6 verify rows stand on the
+    // border: 19.0 us in all, 18.4 with one warp a row)
     const bool many = p.nslot >= kMergeMany || (p.nslot >= 5 && p.hd == 128 && rows <= 4096);
     const int per = kMergeWarps * (p.hd == 64 ? 2 : 1);  // rows of a block
     const dim3 grid((unsigned)((p.hd == 64 || p.hd == 128) && many ? rows : (rows + per - 1) / per));

@@ -228,3 +228,16 @@ def test_own_ranges_that_grow_for_many_rows(kernel):
     got = paged_attention_shared_prefix(q, kv, 0, batch, kernel=kernel)
     _check(got, _exact(q, kv, 0, P, starts), BF)
     kv.check_errors()
+
+
+@pytest.mark.parametrize("case", PLANTS, ids=str)
+def test_rows_of_nothing_but_infinitely_low_scores_are_zero(case):
+    kernel, P, before, chunk, d, bs, dtype = case
+    kv, batch, q, exact, _ = _planted(case, True)
+    q[..., 4:, :] = q[..., 4:, :].abs() + 0.5
+    kv._k[:, :, :, 1] = float("-inf")  # every key of kv head 1
+    kv._v[:, :, :, 1].nan_to_num_(2.0)
+    got = paged_attention_shared_prefix(q, kv, 0, batch, kernel=kernel)
+    assert (got[:, :, 4:] == 0).all()
+    _check(got[:, :, :4], tuple(x[:, :, :4] for x in exact), dtype if dtype != F32 else None)
+    kv.check_errors()
